@@ -258,7 +258,7 @@ int check_page_ranges(void* const* dst, const void* const* src, const int64_t* p
 	for (int64_t i = 0; i < count; ++i)
 	{
 		const uintptr_t at = reinterpret_cast<uintptr_t>(dst[i]);
-		if (dst_pages[i] > 0) written[n++] = {at, at + (uintptr_t)(dst_pages[i] * page_bytes[i])};
+		if (dst_pages[i] > 0 && page_bytes[i] > 0) written[n++] = {at, at + (uintptr_t)(dst_pages[i] * page_bytes[i])};
 	}
 	std::sort(written, written + n, [](const Range& a, const Range& b) { return a.from < b.from; });
 	for (int64_t i = 1; i < n; ++i)
@@ -266,7 +266,7 @@ int check_page_ranges(void* const* dst, const void* const* src, const int64_t* p
 	for (int64_t i = 0; i < count; ++i)
 	{
 		const uintptr_t from = reinterpret_cast<uintptr_t>(src[i]), to = from + (uintptr_t)(src_pages[i] * page_bytes[i]);
-		if (src_pages[i] == 0 || (src[i] == dst[i] && src_pages[i] == dst_pages[i])) continue;
+		if (to == from || (src[i] == dst[i] && src_pages[i] == dst_pages[i])) continue;
 		const Range* const behind = std::lower_bound(written, written + n, from, [](const Range& r, uintptr_t v) { return r.to <= v; });
 		if (behind != written + n && behind->from < to) return ANYGPU_ERR_BAD_SHAPE;
 	}
