@@ -245,13 +245,13 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 		out[L::kInLow * kChunk + lane] = (float)(in - (double)in_hi);
 		if constexpr (HALF)
 		{
-			// exp(-L_s) delta_s as one exponential; a token without a step has no weight
+			// exp(-L_s) delta_s as one exponential; a token without a step, and one whose step is no normal float (the logarithm takes it for none), has no weight
 			const float log_delta = __builtin_amdgcn_logf(delta);
 			const double from = in - (double)log_delta;
 			const float from_hi = (float)from;
 			out[L::kOut * kChunk + lane] = (float)(to_end + (double)log_delta);
 			out[L::kFrom * kChunk + lane] = from_hi;
-			out[L::kFromLow * kChunk + lane] = delta > 0.0f ? (float)(from - (double)from_hi) : 0.0f;
+			out[L::kFromLow * kChunk + lane] = from_hi < INFINITY ? (float)(from - (double)from_hi) : 0.0f;
 		}
 		else
 		{
