@@ -16,7 +16,7 @@
 // what y itself is rounded to; the weights of a token's own tile, which are the largest, keep their remainders.  The state itself stays float32: w x enters
 // as the sum of two halves, 22 bits.  Whether the values that become halves lie where a half has its bits is looked at every time (a maximum and a few lane
 // masks); where they do not, they are brought there by powers of two, which comes out of the sums again.  That path is the slower one by a multiplication per
-// value on either side: the state is kept 2^8 times what it is, which puts common steps and states inside.
+// value on either side: the state is kept 2^8 times what it is, which puts common steps and states inside.  The state goes along only as far as it remains a float.
 // float32: every operand is the sum of two halves, 22 bits and a sign more than a half has, and a product is three (what is left out lies below 2^-24 of it).  x, B
 // and C are scaled by the powers of two that bring a chunk's largest element to the top of a half's range, the state and the weights likewise; sums are
 // float32.  The fp32 matrix instruction does a sixteenth of what the one for halves does in its time (4 x 4096 tokens, 64 heads: 292 us with it, 194 with halves).
@@ -75,7 +75,7 @@ struct Lds
 	// precision), exp(L), weight into the state, delta (float32)
 	static constexpr int kIn = 0, kInLow = 1, kOut = 2, kGain = 3, kWeight = 4, kFrom = 5, kFromLow = 6, kDelta = 5, kArrays = kHalf ? 7 : 6;
 	// and: steps across the four tiles, the chunk's decay; float32: what the scales of x, B and C make of sums (see store_chunk)
-	static constexpr int kDecay = 4, kScaleBC = 5, kScaleXC = 6, kScaleX = 7, kScaleBX = 8;
+	static constexpr int kDecay = 4, kScaleBC = 5, kScaleC = 6, kScaleX = 7, kScaleBX = 8;
 	static constexpr int kSet = kArrays * kChunk * 4 + 48;
 	static constexpr int kMost = kSteps + 2 * kSet;                         // float32: the largest x, B and C of a chunk by wave, two sets
 	static constexpr int kBytes = kMost + (kHalf ? 0 : 2 * 3 * 16);
@@ -92,7 +92,7 @@ __device__ __forceinline__ float power_of_two(int k) { return __builtin_bit_cast
 
 __device__ __forceinline__ void half_scale(float v, float& up, float& down)
 {
-	const int k = half_exponent(v, -100, 58);
+	const int k = half_exponent(v, -113, 58);
 	up = power_of_two(k);
 	down = power_of_two(-k);
 }
@@ -277,9 +277,9 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 		// (without result waves one of these sums up the steps)
 		const bool stepper = STATES && moves && wave == (int)(blockIdx.x & (PT - 1));
 
-		// ---- the state: column p = 16 wave + l, rows n = 16 i + 4 g + r; in units of its own ----
+		// ---- the state: column p = 16 wave + l, rows n = 16 i + 4 g + r; half precision: kUnit times what it is ----
 		float4_t h[NB];
-		float decay = 1.0f, unit = HALF ? 1.0f / kUnit : 1.0f;               // what an element of h is worth (float32: by the scales of the chunk)
+		float decay = 1.0f;
 		const int hp = 16 * wave + l;
 		float* state = a.state + ((int64_t)bh * a.head_dim + p0 + hp) * a.state_row;
 		const bool wide = size % 4 == 0 && a.state_row % 4 == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0;
@@ -465,11 +465,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					for (int k = 1; k < PT; ++k) most = fmaxf(most, m[k]);
 					return most > 0.0f ? half_exponent(most, -60, highest) : 0;
 				};
-				// (those of x and B are the state's as well, which is to fit up to 2^70: 2^56 at most)
-				int k_x = exponent(0, 58), k_b = exponent(1, 80);
-				const int excess = k_x + k_b > 56 ? k_x + k_b - 56 : 0, k_c = STATES ? 0 : exponent(2, 40);
-				k_x -= excess >> 1;
-				k_b -= excess - (excess >> 1);
+				const int k_x = exponent(0, 58), k_b = exponent(1, 80), k_c = STATES ? 0 : exponent(2, 40);
 				up_x = power_of_two(k_x);
 				up_b = power_of_two(k_b);
 				up_c = power_of_two(k_c);
@@ -477,9 +473,9 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				{
 					float* const out = reinterpret_cast<float*>(lds + L::kSteps + set * L::kSet) + L::kArrays * kChunk;
 					out[L::kScaleBC] = kUnit * power_of_two(-k_b) * power_of_two(-k_c);        // products of B and C -> weights, kUnit times what they are
-					out[L::kScaleXC] = kUnit * up_x * power_of_two(-k_c);                      // products of the state and C -> those of x and weights
-					out[L::kScaleX] = 1.0f / kUnit * power_of_two(-k_x);                       // these -> results
-					out[L::kScaleBX] = up_b * up_x;                                          // products of B and x against what they are
+					out[L::kScaleC] = power_of_two(-k_c);                                      // products of the state and C -> results
+					out[L::kScaleX] = 1.0f / kUnit * power_of_two(-k_x);                       // products of x and weights -> results
+					reinterpret_cast<int*>(out)[L::kScaleBX] = -(k_b + k_x);                   // products of B and x -> the state, the exponent
 				}
 			}
 			store_rows(o.x, at + L::kX, L::kPitchX, L::kXLow, up_x, 0);
@@ -551,7 +547,6 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				{
 					float up;
 					half_scale(wave_allreduce(finite_or_zero(most), MaxOp()), up, down);
-					down *= unit;
 #pragma unroll
 					for (int i = 0; i < NB; ++i)
 					{
@@ -695,50 +690,88 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 			}
 			// (below 2^-4 the second half of a value lies among the numbers whose last bit is worth 2^-24, which leaves 21 bits; float32: 24)
 			const bool scaled = rows_need_scale(most, HALF ? 0.0625f : 0.5f);
-			float down = 1.0f, into = keep;
+			float into = keep, down = 1.0f;
+			int back = 0;                                         // float32: 2^back, products -> the state
+			if constexpr (!HALF) back = reinterpret_cast<const int*>(steps)[L::kArrays * kChunk + L::kScaleBX];
 			if (scaled)
 			{
-				float up;
-				half_scale(max_over_lane_rows(most), up, down);
-				into *= up;
+				int k = half_exponent(max_over_lane_rows(most), -113, 58);
+				if constexpr (HALF)
+				{
+					// (the state goes along, as far as it remains a float)
+					float largest = 0.0f;
+#pragma unroll
+					for (int i = 0; i < NB; ++i)
+#pragma unroll
+						for (int r = 0; r < 4; ++r) largest = fmaxf(largest, __builtin_fabsf(h[i][r]));
+					const int room = 252 - ((__builtin_bit_cast(int, max_over_lane_rows(largest)) >> 23) & 255);
+					k = k < room ? k : room;
+					into *= power_of_two(k);
+					down = power_of_two(-k);
+				}
+				else back -= k;
+				const float up = power_of_two(k);
 #pragma unroll
 				for (int q = 0; q < 4; ++q) v[q] = v[q] * up;
 			}
-			if constexpr (!HALF)
-			{
-				const float chunk_scale = steps[L::kArrays * kChunk + L::kScaleBX];
-				into *= fminf(unit * chunk_scale, 0x1p126f);               // (no infinity for a state of zeros)
-				unit = __builtin_bit_cast(float, (254 << 23) - __builtin_bit_cast(int, chunk_scale));      // 1 / a power of two
-			}
-#pragma unroll
-			for (int i = 0; i < NB; ++i) h[i] = h[i] * into;
 			half4_t hi[4], low[4];
 #pragma unroll
 			for (int q = 0; q < 4; ++q) split(v[q], hi[q], low[q]);
-#pragma unroll
-			for (int kk = 0; kk < 2; ++kk)
+			if constexpr (HALF)
 			{
-				const half8_t v_low = join(low[2 * kk], low[2 * kk + 1]), v_hi = join(hi[2 * kk], hi[2 * kk + 1]);
-				const char* const at = ops + L::kB + l * L::kPitchB + (32 * kk + 8 * g) * 2;
-				half8_t bf[NB];
-				if constexpr (!HALF)
-				{
 #pragma unroll
-					for (int i = 0; i < NB; ++i) bf[i] = *reinterpret_cast<const half8_t*>(at + 16 * i * L::kPitchB + L::kBLow);
+				for (int i = 0; i < NB; ++i) h[i] = h[i] * into;
+#pragma unroll
+				for (int kk = 0; kk < 2; ++kk)
+				{
+					const half8_t v_low = join(low[2 * kk], low[2 * kk + 1]), v_hi = join(hi[2 * kk], hi[2 * kk + 1]);
+					const char* const at = ops + L::kB + l * L::kPitchB + (32 * kk + 8 * g) * 2;
+					half8_t bf[NB];
+#pragma unroll
+					for (int i = 0; i < NB; ++i) bf[i] = *reinterpret_cast<const half8_t*>(at + 16 * i * L::kPitchB);
+#pragma unroll
+					for (int i = 0; i < NB; ++i) h[i] = mfma(bf[i], v_low, h[i]);
 #pragma unroll
 					for (int i = 0; i < NB; ++i) h[i] = mfma(bf[i], v_hi, h[i]);
 				}
+				if (scaled)
+				{
 #pragma unroll
-				for (int i = 0; i < NB; ++i) bf[i] = *reinterpret_cast<const half8_t*>(at + 16 * i * L::kPitchB);
-#pragma unroll
-				for (int i = 0; i < NB; ++i) h[i] = mfma(bf[i], v_low, h[i]);
-#pragma unroll
-				for (int i = 0; i < NB; ++i) h[i] = mfma(bf[i], v_hi, h[i]);
+					for (int i = 0; i < NB; ++i) h[i] = h[i] * down;
+				}
 			}
-			if (scaled)
+			else
 			{
+				// sums of their own, two tiles at a time: the state may be far from what enters it, and keeps its range
+				constexpr int TILES = 2;
 #pragma unroll
-				for (int i = 0; i < NB; ++i) h[i] = h[i] * down;
+				for (int i0 = 0; i0 < NB; i0 += TILES)
+				{
+					float4_t sum[TILES];
+#pragma unroll
+					for (int i = 0; i < TILES; ++i) sum[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+					for (int kk = 0; kk < 2; ++kk)
+					{
+						const half8_t v_low = join(low[2 * kk], low[2 * kk + 1]), v_hi = join(hi[2 * kk], hi[2 * kk + 1]);
+						const char* const at = ops + L::kB + (16 * i0 + l) * L::kPitchB + (32 * kk + 8 * g) * 2;
+						half8_t bf[TILES];
+#pragma unroll
+						for (int i = 0; i < TILES; ++i) bf[i] = *reinterpret_cast<const half8_t*>(at + 16 * i * L::kPitchB + L::kBLow);
+#pragma unroll
+						for (int i = 0; i < TILES; ++i) sum[i] = mfma(bf[i], v_hi, sum[i]);
+#pragma unroll
+						for (int i = 0; i < TILES; ++i) bf[i] = *reinterpret_cast<const half8_t*>(at + 16 * i * L::kPitchB);
+#pragma unroll
+						for (int i = 0; i < TILES; ++i) sum[i] = mfma(bf[i], v_low, sum[i]);
+#pragma unroll
+						for (int i = 0; i < TILES; ++i) sum[i] = mfma(bf[i], v_hi, sum[i]);
+					}
+#pragma unroll
+					for (int i = 0; i < TILES; ++i)
+#pragma unroll
+						for (int r = 0; r < 4; ++r) h[i0 + i][r] = fmaf(h[i0 + i][r], keep, __builtin_amdgcn_ldexpf(sum[i][r], back));
+				}
 			}
 			if (more && stepper) make_steps(t0 + kChunk, (float)raw_next, turn ^ 1);
 			if constexpr (DOUBLE)
@@ -760,8 +793,11 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				}
 			}
 		}
+		if constexpr (HALF)
+		{
 #pragma unroll
-		for (int i = 0; i < NB; ++i) h[i] = h[i] * unit;
+			for (int i = 0; i < NB; ++i) h[i] = h[i] * (1.0f / kUnit);
+		}
 		if constexpr (STATES)
 		{
 #pragma unroll
@@ -902,7 +938,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 			{
 				const float* tiles = reinterpret_cast<const float*>(front + L::kTiles);
 #pragma unroll
-				for (int pt = 0; pt < PT; ++pt) into[pt] = tiles[pt] * gain * (HALF ? 1.0f : steps[L::kArrays * kChunk + L::kScaleXC]);
+				for (int pt = 0; pt < PT; ++pt) into[pt] = tiles[pt] * gain * (HALF ? 1.0f : steps[L::kArrays * kChunk + L::kScaleC]);
 			}
 			// (from 2^-9 on what a column's small weights lose is far below a rounding of its largest; the second halves ask for 2^-1)
 			const bool scaled = rows_need_scale(most, HALF ? 0.001953125f : 0.5f);
@@ -911,8 +947,13 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 			{
 				float up, back;
 				half_scale(max_over_lane_rows(most), up, back);
-				into = into * up;
 				down *= back;
+				if constexpr (HALF)
+				{
+					// (no infinity for a state that nobody reads)
+#pragma unroll
+					for (int pt = 0; pt < PT; ++pt) into[pt] = fminf(into[pt] * up, 0x1p127f);
+				}
 #pragma unroll
 				for (int j = 0; j <= TT; ++j) gw[j] = gw[j] * up;
 			}
@@ -932,7 +973,9 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 #pragma unroll
 			for (int pt = 0; pt < PT; ++pt)
 			{
-				acc[pt] = acc[pt] * into[pt];
+				// float32: apart from the state's part, which has a scale of its own.  (In half precision a result that is far from its weights is no half.)
+				float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+				if constexpr (HALF) sum = acc[pt] * into[pt];
 #pragma unroll
 				for (int kk = 0; 2 * kk <= TT; ++kk)
 				{
@@ -944,13 +987,19 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					if constexpr (!HALF)
 					{
 						const half8_t xl = join(*reinterpret_cast<const half4_t*>(row + L::kXLow + x_at[2 * kk]), *reinterpret_cast<const half4_t*>(row + L::kXLow + x_at[2 * kk + 1]));
-						acc[pt] = mfma(xl, w_hi, acc[pt]);
+						sum = mfma(xl, w_hi, sum);
 					}
-					if (!HALF || kk == TT / 2) acc[pt] = mfma(xf, w_low, acc[pt]);
-					acc[pt] = mfma(xf, w_hi, acc[pt]);
+					if (!HALF || kk == TT / 2) sum = mfma(xf, w_low, sum);
+					sum = mfma(xf, w_hi, sum);
+				}
+				if constexpr (HALF) acc[pt] = sum;
+				else
+				{
+#pragma unroll
+					for (int r = 0; r < 4; ++r) acc[pt][r] = fmaf(acc[pt][r], into[pt], sum[r] * down);
 				}
 			}
-			if (!HALF || scaled)
+			if (HALF && scaled)
 			{
 #pragma unroll
 				for (int pt = 0; pt < PT; ++pt) acc[pt] = acc[pt] * down;
