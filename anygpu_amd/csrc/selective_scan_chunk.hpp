@@ -17,9 +17,10 @@
 // as the sum of two halves, 22 bits.  Whether the values that become halves lie where a half has its bits is looked at every time (a maximum and a few lane
 // masks); where they do not, they are brought there by powers of two, which comes out of the sums again.  That path is the slower one by a multiplication per
 // value on either side: the state is kept 2^8 times what it is, which puts common steps and states inside.  The state goes along only as far as it remains a float.
-// float32: every operand is the sum of two halves, 22 bits and a sign more than a half has, and a product is three (what is left out lies below 2^-24 of it).  x, B
-// and C are scaled by the powers of two that bring a chunk's largest element to the top of a half's range, the state and the weights likewise; sums are
-// float32.  The fp32 matrix instruction does a sixteenth of what the one for halves does in its time (4 x 4096 tokens, 64 heads: 292 us with it, 194 with halves).
+// float32: every operand is the sum of two halves, 22 bits and a sign more than a half has, and a product is three (what is left out lies below 2^-22 of it).  The
+// second halves are 2^11 times what they are and their products summed apart, so that they have their bits as far down as the first ones.  x, B
+// and C are scaled by the powers of two that bring a chunk's largest element to the top of a half's range, the state and the weights likewise: all 22 bits down to
+// 2^-29 of the largest, 2^-51 of the largest below that.  Sums are float32, and powers of two come out of them by exponents.  The fp32 matrix instruction does a sixteenth of what the one for halves does in its time (4 x 4096 tokens, 64 heads: 292 us with it, 194 with halves).
 // Steps are summed in 64 bits, and the distance of two tokens is put together from pieces of one sign - from a token to its tile's edge, tile by tile, and
 // from an edge to a token - so that no difference of long sums is taken; inside a tile the sums are pairs of floats.
 //
@@ -39,7 +40,7 @@ namespace anygpu {
 namespace scan {
 
 constexpr int kChunk = 64;                  // tokens
-constexpr float kUnit = 256.0f;             // the state and the weights into it (half precision), the weights of the results (float32) are kept this many times what they are
+constexpr float kUnit = 256.0f;             // half precision: the state and the weights into it are kept this many times what they are
 
 // Where the sequences are shared out in segments: a first launch leaves the state behind every part of the segments but the last (taken from zeros, the first one's
 // from the given state) and the decay across it, the second starts every segment from what the parts before it leave.
@@ -74,8 +75,8 @@ struct Lds
 	// of a token: steps since its tile's start (pair), the same less log2(delta) (half precision, pair), from it to its tile's end (+ log2(delta) in half
 	// precision), exp(L), weight into the state, delta (float32)
 	static constexpr int kIn = 0, kInLow = 1, kOut = 2, kGain = 3, kWeight = 4, kFrom = 5, kFromLow = 6, kDelta = 5, kArrays = kHalf ? 7 : 6;
-	// and: steps across the four tiles, the chunk's decay; float32: what the scales of x, B and C make of sums (see store_chunk)
-	static constexpr int kDecay = 4, kScaleBC = 5, kScaleC = 6, kScaleX = 7, kScaleBX = 8;
+	// and: steps across the four tiles, the chunk's decay; float32: what the scales of x, B and C make of sums (see store_chunk; kBack: exponents)
+	static constexpr int kDecay = 4, kScaleBC = 5, kSkip = 6, kBackX = 7, kBackC = 8, kBackBX = 9;
 	static constexpr int kSet = kArrays * kChunk * 4 + 48;
 	static constexpr int kMost = kSteps + 2 * kSet;                         // float32: the largest x, B and C of a chunk by wave, two sets
 	static constexpr int kBytes = kMost + (kHalf ? 0 : 2 * 3 * 16);
@@ -88,11 +89,13 @@ __device__ __forceinline__ int half_exponent(float v, int lowest, int highest)
 	return k < lowest ? lowest : k > highest ? highest : k;
 }
 
+constexpr int kLowest = -113, kHighest = 116;       // of the largest float, and of what is a float 2^11 times as large
+
 __device__ __forceinline__ float power_of_two(int k) { return __builtin_bit_cast(float, (127 + k) << 23); }
 
 __device__ __forceinline__ void half_scale(float v, float& up, float& down)
 {
-	const int k = half_exponent(v, -113, 58);
+	const int k = half_exponent(v, kLowest, 58);
 	up = power_of_two(k);
 	down = power_of_two(-k);
 }
@@ -172,6 +175,25 @@ __device__ __forceinline__ double read_lane_f64(double v, int lane)
 	return __builtin_bit_cast(double, p);
 }
 
+// The same with the remainders 2^11 times what they are: as far above the smallest half as the values themselves.  Products with them are summed apart.
+constexpr float kLowUnit = 2048.0f;
+
+__device__ __forceinline__ void split_wide(float4_t v, half4_t& hi, half4_t& low)
+{
+	hi = __builtin_convertvector(v, half4_t);
+	const half2_t h0 = {hi[0], hi[1]}, h1 = {hi[2], hi[3]};
+	const float4_t rest = {remainder_of<0>(v[0], h0), remainder_of<1>(v[1], h0), remainder_of<0>(v[2], h1), remainder_of<1>(v[3], h1)};
+	low = __builtin_convertvector(rest * kLowUnit, half4_t);
+}
+
+__device__ __forceinline__ float4_t add_low(float4_t main, float4_t low)
+{
+	float4_t r;
+#pragma unroll
+	for (int i = 0; i < 4; ++i) r[i] = fmaf(low[i], 1.0f / kLowUnit, main[i]);
+	return r;
+}
+
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
 // (lane i of a group of 16 gets element i of the 4-row band whose row i / 4, columns 4 (i % 4) .. + 3 its address points at)
@@ -222,7 +244,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 
 	const T* dt = static_cast<const T*>(a.dt) + batch * a.dt_batch + head * a.dt_head;
 	const double rate = (double)a.a[head] * 1.4426950408889634;
-	const float bias = a.bias ? a.bias[head] : 0.0f;
+	const float bias = a.bias ? a.bias[head] : 0.0f, skip = a.skip ? a.skip[head] : 0.0f;
 	const auto load_step = [&](int t0) { return dt[(t0 + lane < end ? t0 + lane : end - 1) * a.dt_seq]; };
 	// a chunk's sums of steps, a token per lane of one wave
 	const auto make_steps = [&](int t0, float raw, int set) {
@@ -403,8 +425,12 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				for (int i = 0; i < BA; ++i) o.b[i] = *fetch(b + t0, bo[i]);
 				if constexpr (!STATES)
 				{
+					// (float32 without waves that only fetch: 256 registers are all there are, and C's offsets are made afresh - 66.5 us instead of 68.2 with a spilled pair of them
+					// for 3 x 1001 tokens, 32 heads, state 128)
+					unsigned c_row = (unsigned)a.c_row;
+					if constexpr (!HALF && !MOVERS) asm volatile("" : "+s"(c_row));
 #pragma unroll
-					for (int i = 0; i < BA; ++i) o.c[i] = *fetch(c + t0, co[i]);
+					for (int i = 0; i < BA; ++i) o.c[i] = *fetch(c + t0, HALF || MOVERS ? co[i] : offset(i, size, c_row));
 				}
 			}
 		};
@@ -419,9 +445,9 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					for (int i = 0; i < COUNT; ++i)
 #pragma unroll
 						for (int e = 0; e < 4; ++e) m = fmaxf(m, __builtin_fabsf(v[i][e]));
-					// Between 2^-6 and 2^7 they are given as 2^6, a scale of 2^8: no reduction over the wave, and what is left of its bits is 2^-33
-						float noted = 64.0f;
-					if (__builtin_amdgcn_ballot_w64(!(m < 128.0f)) != 0 || __builtin_amdgcn_ballot_w64(m >= 0.015625f) == 0)
+					// Between 1 and 2^7 they are given as 2^6, a scale of 2^8: no reduction over the wave, and what two halves leave there is 2^-44
+					float noted = 64.0f;
+					if (__builtin_amdgcn_ballot_w64(!(m < 128.0f)) != 0 || __builtin_amdgcn_ballot_w64(m >= 1.0f) == 0)
 					{
 						m = 0.0f;
 #pragma unroll
@@ -447,7 +473,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				else
 				{
 					half4_t first, second;
-					split(v[i] * up, first, second);
+					split_wide(v[i] * up, first, second);
 					*reinterpret_cast<half4_t*>(to) = first;
 					*reinterpret_cast<half4_t*>(to + low) = second;
 				}
@@ -463,19 +489,30 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					float most = m[0];
 #pragma unroll
 					for (int k = 1; k < PT; ++k) most = fmaxf(most, m[k]);
-					return most > 0.0f ? half_exponent(most, -60, highest) : 0;
+					return most > 0.0f ? half_exponent(most, kLowest, highest) : 0;
 				};
-				const int k_x = exponent(0, 58), k_b = exponent(1, 80), k_c = STATES ? 0 : exponent(2, 40);
+				// (2^126 for B and C together: what their products become as weights is to be a float)
+				const int k_x = exponent(0, kHighest);
+				int k_b = exponent(1, kHighest), k_c = STATES ? 0 : exponent(2, kHighest);
+				const int excess = k_b + k_c > 126 ? k_b + k_c - 126 : 0;
+				k_b -= excess >> 1;
+				k_c -= excess - (excess >> 1);
 				up_x = power_of_two(k_x);
 				up_b = power_of_two(k_b);
 				up_c = power_of_two(k_c);
 				if (tid == 0)
 				{
 					float* const out = reinterpret_cast<float*>(lds + L::kSteps + set * L::kSet) + L::kArrays * kChunk;
-					out[L::kScaleBC] = kUnit * power_of_two(-k_b) * power_of_two(-k_c);        // products of B and C -> weights, kUnit times what they are
-					out[L::kScaleC] = power_of_two(-k_c);                                      // products of the state and C -> results
-					out[L::kScaleX] = 1.0f / kUnit * power_of_two(-k_x);                       // products of x and weights -> results
-					reinterpret_cast<int*>(out)[L::kScaleBX] = -(k_b + k_x);                   // products of B and x -> the state, the exponent
+					int* const back = reinterpret_cast<int*>(out);
+					// The products of B and C are up to 2^38; as weights they are 2^30 times less, and less than that where D would not be a float of their unit.
+					const int skip_exponent = ((__builtin_bit_cast(int, skip) >> 23) & 255) - 126, room = 100 - (skip_exponent > 0 ? skip_exponent : 0);
+					int unit = k_b + k_c - 30 < room ? k_b + k_c - 30 : room;
+					unit = unit > k_b + k_c - 126 ? unit : k_b + k_c - 126;
+					out[L::kScaleBC] = power_of_two(unit - k_b - k_c);                       // products of B and C -> weights, 2^unit times what they are
+					out[L::kSkip] = __builtin_amdgcn_ldexpf(skip, unit);
+					back[L::kBackX] = -(unit + k_x);                                         // products of x and weights -> results
+					back[L::kBackC] = -k_c;                                                  // products of the state and C -> results
+					back[L::kBackBX] = -(k_b + k_x);                                         // products of B and x -> the state
 				}
 			}
 			store_rows(o.x, at + L::kX, L::kPitchX, L::kXLow, up_x, 0);
@@ -520,7 +557,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				for (int i = 0; i < NB; ++i)
 #pragma unroll
 					for (int r = 0; r < 4; ++r) most = fmaxf(most, __builtin_fabsf(h[i][r]));
-				float down = 1.0f;
+				float down = 1.0f;                                   // (float32: the exponent)
 				if constexpr (HALF)
 				{
 					// one scale for the wave's rows: they fit, and the largest element has bits to spare for rows with smaller ones
@@ -545,13 +582,14 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				}
 				else
 				{
-					float up;
-					half_scale(wave_allreduce(finite_or_zero(most), MaxOp()), up, down);
+					const int k = half_exponent(wave_allreduce(finite_or_zero(most), MaxOp()), kLowest, kHighest);
+					const float up = power_of_two(k);
+					down = __builtin_bit_cast(float, -k);
 #pragma unroll
 					for (int i = 0; i < NB; ++i)
 					{
 						half4_t first, second;
-						split(h[i] * up, first, second);
+						split_wide(h[i] * up, first, second);
 						*reinterpret_cast<half4_t*>(row + (16 * i + 4 * g) * 2) = first;
 						*reinterpret_cast<half4_t*>(row + L::kHLow + (16 * i + 4 * g) * 2) = second;
 					}
@@ -681,22 +719,22 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					if constexpr (!HALF)
 					{
 						const half2_t y0 = {xl[4 * q], xl[4 * q + 1]}, y1 = {xl[4 * q + 2], xl[4 * q + 3]};
-						u = float4_t{times_half_add<0>(y0, w[0], u[0]), times_half_add<1>(y0, w[1], u[1]), times_half_add<0>(y1, w[2], u[2]), times_half_add<1>(y1, w[3], u[3])};
+						const float4_t w_low = w * (1.0f / kLowUnit);
+						u = float4_t{times_half_add<0>(y0, w_low[0], u[0]), times_half_add<1>(y0, w_low[1], u[1]), times_half_add<0>(y1, w_low[2], u[2]), times_half_add<1>(y1, w_low[3], u[3])};
 					}
 					v[2 * kk + q] = u;
 #pragma unroll
 					for (int e = 0; e < 4; ++e) most = fmaxf(most, __builtin_fabsf(u[e]));
 				}
 			}
-			// (below 2^-4 the second half of a value lies among the numbers whose last bit is worth 2^-24, which leaves 21 bits; float32: 24)
-			const bool scaled = rows_need_scale(most, HALF ? 0.0625f : 0.5f);
 			float into = keep, down = 1.0f;
+			bool scaled = false;
 			int back = 0;                                         // float32: 2^back, products -> the state
-			if constexpr (!HALF) back = reinterpret_cast<const int*>(steps)[L::kArrays * kChunk + L::kScaleBX];
-			if (scaled)
+			if constexpr (HALF)
 			{
-				int k = half_exponent(max_over_lane_rows(most), -113, 58);
-				if constexpr (HALF)
+				// (below 2^-4 the second half of a value lies among the numbers whose last bit is worth 2^-24, which leaves 21 bits)
+				scaled = rows_need_scale(most, 0.0625f);
+				if (scaled)
 				{
 					// (the state goes along, as far as it remains a float)
 					float largest = 0.0f;
@@ -704,19 +742,30 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					for (int i = 0; i < NB; ++i)
 #pragma unroll
 						for (int r = 0; r < 4; ++r) largest = fmaxf(largest, __builtin_fabsf(h[i][r]));
-					const int room = 252 - ((__builtin_bit_cast(int, max_over_lane_rows(largest)) >> 23) & 255);
-					k = k < room ? k : room;
-					into *= power_of_two(k);
+					const int k_most = half_exponent(max_over_lane_rows(most), kLowest, 58),
+					          room = 252 - ((__builtin_bit_cast(int, max_over_lane_rows(largest)) >> 23) & 255), k = k_most < room ? k_most : room;
+					const float up = power_of_two(k);
+					into *= up;
 					down = power_of_two(-k);
+#pragma unroll
+					for (int q = 0; q < 4; ++q) v[q] = v[q] * up;
 				}
-				else back -= k;
+			}
+			else
+			{
+				const int k = half_exponent(max_over_lane_rows(most), kLowest, kHighest);
 				const float up = power_of_two(k);
+				back = reinterpret_cast<const int*>(steps)[L::kArrays * kChunk + L::kBackBX] - k;
 #pragma unroll
 				for (int q = 0; q < 4; ++q) v[q] = v[q] * up;
 			}
 			half4_t hi[4], low[4];
 #pragma unroll
-			for (int q = 0; q < 4; ++q) split(v[q], hi[q], low[q]);
+			for (int q = 0; q < 4; ++q)
+			{
+				if constexpr (HALF) split(v[q], hi[q], low[q]);
+				else split_wide(v[q], hi[q], low[q]);
+			}
 			if constexpr (HALF)
 			{
 #pragma unroll
@@ -747,9 +796,9 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 #pragma unroll
 				for (int i0 = 0; i0 < NB; i0 += TILES)
 				{
-					float4_t sum[TILES];
+					float4_t sum[TILES], low_sum[TILES];
 #pragma unroll
-					for (int i = 0; i < TILES; ++i) sum[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+					for (int i = 0; i < TILES; ++i) sum[i] = low_sum[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
 					for (int kk = 0; kk < 2; ++kk)
 					{
@@ -759,18 +808,21 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 #pragma unroll
 						for (int i = 0; i < TILES; ++i) bf[i] = *reinterpret_cast<const half8_t*>(at + 16 * i * L::kPitchB + L::kBLow);
 #pragma unroll
-						for (int i = 0; i < TILES; ++i) sum[i] = mfma(bf[i], v_hi, sum[i]);
+						for (int i = 0; i < TILES; ++i) low_sum[i] = mfma(bf[i], v_hi, low_sum[i]);
 #pragma unroll
 						for (int i = 0; i < TILES; ++i) bf[i] = *reinterpret_cast<const half8_t*>(at + 16 * i * L::kPitchB);
 #pragma unroll
-						for (int i = 0; i < TILES; ++i) sum[i] = mfma(bf[i], v_low, sum[i]);
+						for (int i = 0; i < TILES; ++i) low_sum[i] = mfma(bf[i], v_low, low_sum[i]);
 #pragma unroll
 						for (int i = 0; i < TILES; ++i) sum[i] = mfma(bf[i], v_hi, sum[i]);
 					}
 #pragma unroll
 					for (int i = 0; i < TILES; ++i)
+					{
+						const float4_t both = add_low(sum[i], low_sum[i]);
 #pragma unroll
-						for (int r = 0; r < 4; ++r) h[i0 + i][r] = fmaf(h[i0 + i][r], keep, __builtin_amdgcn_ldexpf(sum[i][r], back));
+						for (int r = 0; r < 4; ++r) h[i0 + i][r] = fmaf(h[i0 + i][r], keep, __builtin_amdgcn_ldexpf(both[r], back));
+					}
 				}
 			}
 			if (more && stepper) make_steps(t0 + kChunk, (float)raw_next, turn ^ 1);
@@ -824,7 +876,6 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 
 	if constexpr (!STATES)
 	{
-		const float skip = a.skip ? a.skip[head] : 0.0f;
 		T* y = static_cast<T*>(a.y) + ((int64_t)batch * a.seqlen * a.heads + head) * a.head_dim + p0;
 		const int64_t y_token = (int64_t)a.heads * a.head_dim;
 		// the waves of a block have one to four tiles of weights each; blocks deal them out differently, so that no SIMD has all the long ones
@@ -851,7 +902,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 		for (int r = 0; r < 4; ++r)
 		{
 			behind[r] = 4 * g + r > l ? -INFINITY : 0.0f;
-			itself[r] = 4 * g + r == l ? (HALF ? skip : skip * kUnit) : 0.0f;
+			itself[r] = 4 * g + r == l ? (HALF ? skip : 1.0f) : 0.0f;
 		}
 		const auto chunk = [&](auto which, int t0, int turn, auto before_stores) {
 			constexpr int TT = decltype(which)::value;
@@ -875,6 +926,8 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 			}
 #pragma unroll
 			for (int j = 0; j <= TT; ++j)
+			{
+				float4_t low_sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
 				for (int q = 0; q < NT / 32; ++q)
 				{
@@ -883,13 +936,17 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					if constexpr (!HALF)
 					{
 						const half8_t bl = join(read_transposed(src + L::kBLow), read_transposed(src + L::kBLow + 16 * L::kPitchB));
-						gw[j] = mfma(bl, cf[q], gw[j]);
-						gw[j] = mfma(bf, cl[q], gw[j]);
+						low_sum = mfma(bl, cf[q], low_sum);
+						low_sum = mfma(bf, cl[q], low_sum);
 					}
 					gw[j] = mfma(bf, cf[q], gw[j]);
 				}
+				if constexpr (!HALF) gw[j] = add_low(gw[j], low_sum);
+			}
 #pragma unroll
 			for (int pt = 0; pt < PT; ++pt)
+			{
+				float4_t low_sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
 				for (int q = 0; q < NT / 32; ++q)
 				{
@@ -898,13 +955,16 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					if constexpr (!HALF)
 					{
 						const half8_t hl = join(*reinterpret_cast<const half4_t*>(row + L::kHLow + h_at[2 * q]), *reinterpret_cast<const half4_t*>(row + L::kHLow + h_at[2 * q + 1]));
-						acc[pt] = mfma(hl, cf[q], acc[pt]);
-						acc[pt] = mfma(hf, cl[q], acc[pt]);
+						low_sum = mfma(hl, cf[q], low_sum);
+						low_sum = mfma(hf, cl[q], low_sum);
 					}
 					acc[pt] = mfma(hf, cf[q], acc[pt]);
 				}
+				if constexpr (!HALF) acc[pt] = add_low(acc[pt], low_sum);
+			}
 			// ---- weights: G exp(L_t - L_s) delta_s, the skip term on the diagonal ----
 			const float in = steps[L::kIn * kChunk + t], in_low = steps[L::kInLow * kChunk + t], gain = steps[L::kGain * kChunk + t];
+			const float own = HALF ? 1.0f : steps[L::kArrays * kChunk + L::kSkip];
 			float since = in;                                // from the end of the tile j to the token
 			float most = 0.0f;
 #pragma unroll
@@ -930,30 +990,40 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 #pragma unroll
 				for (int r = 0; r < 4; ++r)
 				{
-					gw[j][r] = j == TT ? fmaf(gw[j][r], e[r], itself[r]) : gw[j][r] * e[r];
+					gw[j][r] = j == TT ? fmaf(gw[j][r], e[r], HALF ? itself[r] : itself[r] * own) : gw[j][r] * e[r];
 					most = fmaxf(most, __builtin_fabsf(gw[j][r]));
 				}
 			}
-			float4_t into;
+			const float* tiles = reinterpret_cast<const float*>(front + L::kTiles);
+			float4_t into;                                   // products of the state and C -> results
+			int into_back[PT], down_back = 0;                // float32: exponents of what the products with C and with the weights are worth
+			float down = 1.0f;
+			bool scaled = false;
+			if constexpr (HALF)
 			{
-				const float* tiles = reinterpret_cast<const float*>(front + L::kTiles);
 #pragma unroll
-				for (int pt = 0; pt < PT; ++pt) into[pt] = tiles[pt] * gain * (HALF ? 1.0f : steps[L::kArrays * kChunk + L::kScaleC]);
-			}
-			// (from 2^-9 on what a column's small weights lose is far below a rounding of its largest; the second halves ask for 2^-1)
-			const bool scaled = rows_need_scale(most, HALF ? 0.001953125f : 0.5f);
-			float down = HALF ? 1.0f : steps[L::kArrays * kChunk + L::kScaleX];
-			if (scaled)
-			{
-				float up, back;
-				half_scale(max_over_lane_rows(most), up, back);
-				down *= back;
-				if constexpr (HALF)
+				for (int pt = 0; pt < PT; ++pt) into[pt] = tiles[pt] * gain;
+				// (from 2^-9 on what a column's small weights lose is far below a rounding of its largest)
+				scaled = rows_need_scale(most, 0.001953125f);
+				if (scaled)
 				{
+					float up;
+					half_scale(max_over_lane_rows(most), up, down);
 					// (no infinity for a state that nobody reads)
 #pragma unroll
 					for (int pt = 0; pt < PT; ++pt) into[pt] = fminf(into[pt] * up, 0x1p127f);
+#pragma unroll
+					for (int j = 0; j <= TT; ++j) gw[j] = gw[j] * up;
 				}
+			}
+			else
+			{
+				const int* const back = reinterpret_cast<const int*>(steps) + L::kArrays * kChunk;
+				const int k = half_exponent(max_over_lane_rows(most), kLowest, kHighest), back_c = back[L::kBackC];
+#pragma unroll
+				for (int pt = 0; pt < PT; ++pt) into_back[pt] = __builtin_bit_cast(int, tiles[pt]) + back_c;
+				down_back = back[L::kBackX] - k;
+				const float up = power_of_two(k);
 #pragma unroll
 				for (int j = 0; j <= TT; ++j) gw[j] = gw[j] * up;
 			}
@@ -968,13 +1038,14 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					wf[j] = __builtin_convertvector(gw[j], half4_t);
 					wl[j] = none;
 				}
-				else split(gw[j], wf[j], wl[j]);
+				else if constexpr (HALF) split(gw[j], wf[j], wl[j]);
+				else split_wide(gw[j], wf[j], wl[j]);
 			}
 #pragma unroll
 			for (int pt = 0; pt < PT; ++pt)
 			{
 				// float32: apart from the state's part, which has a scale of its own.  (In half precision a result that is far from its weights is no half.)
-				float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+				float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f}, low_sum = sum;
 				if constexpr (HALF) sum = acc[pt] * into[pt];
 #pragma unroll
 				for (int kk = 0; 2 * kk <= TT; ++kk)
@@ -987,16 +1058,19 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					if constexpr (!HALF)
 					{
 						const half8_t xl = join(*reinterpret_cast<const half4_t*>(row + L::kXLow + x_at[2 * kk]), *reinterpret_cast<const half4_t*>(row + L::kXLow + x_at[2 * kk + 1]));
-						sum = mfma(xl, w_hi, sum);
+						low_sum = mfma(xl, w_hi, low_sum);
+						low_sum = mfma(xf, w_low, low_sum);
 					}
-					if (!HALF || kk == TT / 2) sum = mfma(xf, w_low, sum);
+					else if (kk == TT / 2) sum = mfma(xf, w_low, sum);
 					sum = mfma(xf, w_hi, sum);
 				}
 				if constexpr (HALF) acc[pt] = sum;
 				else
 				{
+					sum = add_low(sum, low_sum);
 #pragma unroll
-					for (int r = 0; r < 4; ++r) acc[pt][r] = fmaf(acc[pt][r], into[pt], sum[r] * down);
+					for (int r = 0; r < 4; ++r)
+						acc[pt][r] = fmaf(__builtin_amdgcn_ldexpf(acc[pt][r], into_back[pt]), gain, __builtin_amdgcn_ldexpf(sum[r], down_back));
 				}
 			}
 			if (HALF && scaled)

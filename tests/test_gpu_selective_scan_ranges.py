@@ -7,7 +7,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from scan_reference import check_scan, magnitudes, selective_scan  # noqa: E402
+from scan_reference import check_scan, magnitudes, relative, selective_scan  # noqa: E402
 from test_gpu_selective_scan import make, scan  # noqa: E402
 
 
@@ -63,3 +63,82 @@ def test_tokens_without_weights(ops, dtype, much):
     f32 = (4 * 70 + 64 + 16) * 2.0 ** -24
     assert float(((y.double() - want).abs() / (f32 * mag + 2.0 ** -126 * undecayed + 2.0 ** -149)).max()) <= 1.0
     assert float(((state.double() - want_state).abs() / (f32 * mag_state + 2.0 ** -126 * args["state"].double().abs() + 1e-37)).max()) <= 1.0
+
+
+def rows_apart(t, dim, low):
+    """t times factors from 1 down to `low` along the axis, every sixteenth row the same"""
+    n = t.shape[dim]
+    shape = [1] * t.dim()
+    shape[dim] = n
+    return t * torch.logspace(0.0, math.log10(low), 16, device="cuda").repeat(-(-n // 16))[:n].reshape(shape)
+
+
+# Two halves leave 2^-22 of an operand at most, and a product of two pairs leaves out 2^-22: of a term (B C) weight x eight such errors at most (three operands, the
+# weight, three products, exponential and step together).  They are spread evenly and are no one's fault together: eight of 2^-22 / sqrt(3) each add up to 1.7 * 2^-22 in
+# the 2-norm, of results whose 2-norm is that of their terms, for these have no sign in common.  2^-20 leaves a factor of two.
+F32 = 2.0 ** -20
+
+
+@pytest.mark.parametrize("largest", [0.02, 0.1, 1.0, 30.0, 1e4])
+@pytest.mark.parametrize("low", [1e-3, 1e-5, 1e-7])
+@pytest.mark.parametrize("size,seq", [(64, 20), (64, 130), (128, 70), (64, 1500)])
+def test_quiet_channels_in_float32(ops, largest, low, size, seq):
+    args = make("f32", 1, 2, 64, 1, size, seq, carried=False)
+    args["x"] = rows_apart(args["x"] / args["x"].abs().max(), 2, low) * largest
+    args["state"] = torch.zeros(1, 2, 64, size, device="cuda")
+    y, state = scan(ops, args)
+    check_scan(y, state, args)
+    want, want_state = selective_scan(**args)
+    for p in range(64):
+        assert relative(y[..., p], want[..., p]) <= F32, p
+        assert relative(state[:, :, p], want_state[:, :, p]) <= F32, p
+
+
+@pytest.mark.parametrize("key", ["b", "c"])
+@pytest.mark.parametrize("largest", [0.02, 0.1, 1.0, 30.0])
+@pytest.mark.parametrize("low", [1e-3, 1e-5, 1e-7])
+@pytest.mark.parametrize("seq", [20, 130])
+def test_quiet_elements_of_the_state_in_float32(ops, key, largest, low, seq):
+    args = make("f32", 1, 2, 64, 1, 64, seq, carried=False)
+    args[key] = rows_apart(args[key] / args[key].abs().max(), 2, low) * largest
+    # (the other one makes up for it, so that every element counts in a result)
+    other = "c" if key == "b" else "b"
+    args[other] = rows_apart(args[other], 2, 1.0 / low)
+    args["state"] = torch.zeros(1, 2, 64, 64, device="cuda")
+    y, state = scan(ops, args)
+    check_scan(y, state, args)
+    want, want_state = selective_scan(**args)
+    assert relative(y, want) <= F32
+    for n in range(64):
+        assert relative(state[..., n], want_state[..., n]) <= F32, n
+
+
+@pytest.mark.parametrize("key", ["x", "b", "c"])
+@pytest.mark.parametrize("much", [1e4, 1e6, 1e8])
+@pytest.mark.parametrize("size", [64, 128, 200])
+def test_a_loud_token_in_float32(ops, key, much, size):
+    # the tokens in front of it know nothing of it
+    args = make("f32", 1, 2, 64, 1, size, 100)
+    args[key] = args[key].clone()
+    args[key][..., 50] *= much
+    y, state = scan(ops, args)
+    check_scan(y, state, args)
+    want, _ = selective_scan(**args)
+    mag, _ = magnitudes(**args)
+    # (against the terms' magnitudes: all channels of a token share its weights, whose own sums over the state may cancel for all of them alike)
+    for t in range(50):
+        assert float((y[:, t].double() - want[:, t]).norm() / mag[:, t].norm()) <= F32, t
+
+
+@pytest.mark.parametrize("scale_x,scale_b,scale_c", [(1e-30, 1.0, 1.0), (1e30, 1.0, 1.0), (1e37, 1e-20, 1.0), (1e-18, 1e-15, 1e20), (1e25, 1e-20, 1e20), (1.0, 1e-17, 1e17), (1e35, 1e-10, 1e-10),
+                                                    (1.0, 1e30, 1e-30), (1e-5, 1e-20, 1e30)])
+@pytest.mark.parametrize("seq", [100, 1500])
+def test_the_whole_range_of_float32(ops, scale_x, scale_b, scale_c, seq):
+    args = make("f32", 1, 2, 64, 1, 64, seq, carried=False)
+    args.update(x=args["x"] * scale_x, b=args["b"] * scale_b, c=args["c"] * scale_c, state=torch.zeros(1, 2, 64, 64, device="cuda"))
+    if scale_x * scale_b * scale_c > 1e-3 * scale_x:
+        args["skip"] = None
+    y, state = scan(ops, args)
+    want, want_state = selective_scan(**args)
+    assert relative(y, want) <= F32 and relative(state, want_state) <= F32
+    check_scan(y, state, args)
