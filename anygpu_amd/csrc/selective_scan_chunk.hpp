@@ -62,7 +62,8 @@ struct Lds
 	static constexpr int kPitchX = kChunk * 2 + 16, kPitchB = kChunk * 2 + 32, kPitchH = NT * 2 + 16;
 	static constexpr int kXLow = R * kPitchX, kBLow = NT * kPitchB, kHLow = R * kPitchH;       // from the first half to the second
 	static constexpr int kX = 0, kB = kX + kParts * kXLow, kC = kB + kParts * kBLow, kStage = STATES ? kC : kC + kParts * kBLow;
-	static constexpr int kTiles = kParts * kHLow, kFront = STATES ? 0 : kTiles + 16;     // a state in front of a chunk, and the scales of its four tiles
+	// a state in front of a chunk; the scales of four of its rows lie behind each of the first R / 4 rows, in what the pitch leaves there
+	static constexpr int kScales = NT * 2, kFront = STATES ? 0 : kParts * kHLow;
 	static constexpr int kTwoSteps = 2 * 7 * kChunk * 4 + 256;
 	// two chunks' operands where that leaves room for as many blocks as the registers do (half precision: two, three without results) or does not matter
 	static constexpr int kBlocks = kHalf && NT <= 64 ? (STATES ? 3 : 2) : 1;
@@ -557,44 +558,24 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				for (int i = 0; i < NB; ++i)
 #pragma unroll
 					for (int r = 0; r < 4; ++r) most = fmaxf(most, __builtin_fabsf(h[i][r]));
-				float down = 1.0f;                                   // (float32: the exponent)
-				if constexpr (HALF)
-				{
-					// one scale for the wave's rows: they fit, and the largest element has bits to spare for rows with smaller ones
-					const bool fits = __builtin_amdgcn_ballot_w64(!(most < 65504.0f)) == 0 &&
-					                  (__builtin_amdgcn_ballot_w64(most >= 1.0f) != 0 || __builtin_amdgcn_ballot_w64(most > 0.0f) == 0);
-					half4_t out[NB];
-					if (fits)
-					{
+				// a scale for every row, which is a sequence of its own
+				const int k = half_exponent(max_over_lane_rows(most), kLowest, HALF ? 112 : kHighest);
+				const float up = power_of_two(k);
 #pragma unroll
-						for (int i = 0; i < NB; ++i) out[i] = __builtin_convertvector(h[i], half4_t);
-					}
+				for (int i = 0; i < NB; ++i)
+				{
+					char* const at = row + (16 * i + 4 * g) * 2;
+					if constexpr (HALF) *reinterpret_cast<half4_t*>(at) = __builtin_convertvector(h[i] * up, half4_t);
 					else
-					{
-						float up;
-						half_scale(wave_allreduce(finite_or_zero(most), MaxOp()), up, down);
-#pragma unroll
-						for (int i = 0; i < NB; ++i) out[i] = __builtin_convertvector(h[i] * up, half4_t);
-					}
-#pragma unroll
-					for (int i = 0; i < NB; ++i) *reinterpret_cast<half4_t*>(row + (16 * i + 4 * g) * 2) = out[i];
-					down *= 1.0f / kUnit;
-				}
-				else
-				{
-					const int k = half_exponent(wave_allreduce(finite_or_zero(most), MaxOp()), kLowest, kHighest);
-					const float up = power_of_two(k);
-					down = __builtin_bit_cast(float, -k);
-#pragma unroll
-					for (int i = 0; i < NB; ++i)
 					{
 						half4_t first, second;
 						split_wide(h[i] * up, first, second);
-						*reinterpret_cast<half4_t*>(row + (16 * i + 4 * g) * 2) = first;
-						*reinterpret_cast<half4_t*>(row + L::kHLow + (16 * i + 4 * g) * 2) = second;
+						*reinterpret_cast<half4_t*>(at) = first;
+						*reinterpret_cast<half4_t*>(at + L::kHLow) = second;
 					}
 				}
-				if (lane == 0) reinterpret_cast<float*>(to + L::kTiles)[wave] = down;
+				// what a row's products are worth: a factor, in float32 an exponent
+				if (g == 0) *reinterpret_cast<int*>(to + (hp >> 2) * L::kPitchH + L::kScales + (hp & 3) * 4) = HALF ? __builtin_bit_cast(int, power_of_two(-k) * (1.0f / kUnit)) : -k;
 			}
 		};
 		if constexpr (HALF)
@@ -994,24 +975,18 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					most = fmaxf(most, __builtin_fabsf(gw[j][r]));
 				}
 			}
-			const float* tiles = reinterpret_cast<const float*>(front + L::kTiles);
-			float4_t into;                                   // products of the state and C -> results
-			int into_back[PT], down_back = 0;                // float32: exponents of what the products with C and with the weights are worth
-			float down = 1.0f;
+			int back_c = 0, back_w = 0;                      // float32: exponents of what the products with C and with the weights are worth
+			float into = gain, down = 1.0f;                  // products of the state and C -> those with the weights -> results
 			bool scaled = false;
 			if constexpr (HALF)
 			{
-#pragma unroll
-				for (int pt = 0; pt < PT; ++pt) into[pt] = tiles[pt] * gain;
 				// (from 2^-9 on what a column's small weights lose is far below a rounding of its largest)
 				scaled = rows_need_scale(most, 0.001953125f);
 				if (scaled)
 				{
 					float up;
 					half_scale(max_over_lane_rows(most), up, down);
-					// (no infinity for a state that nobody reads)
-#pragma unroll
-					for (int pt = 0; pt < PT; ++pt) into[pt] = fminf(into[pt] * up, 0x1p127f);
+					into *= up;
 #pragma unroll
 					for (int j = 0; j <= TT; ++j) gw[j] = gw[j] * up;
 				}
@@ -1019,10 +994,9 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 			else
 			{
 				const int* const back = reinterpret_cast<const int*>(steps) + L::kArrays * kChunk;
-				const int k = half_exponent(max_over_lane_rows(most), kLowest, kHighest), back_c = back[L::kBackC];
-#pragma unroll
-				for (int pt = 0; pt < PT; ++pt) into_back[pt] = __builtin_bit_cast(int, tiles[pt]) + back_c;
-				down_back = back[L::kBackX] - k;
+				const int k = half_exponent(max_over_lane_rows(most), kLowest, kHighest);
+				back_c = back[L::kBackC];
+				back_w = back[L::kBackX] - k;
 				const float up = power_of_two(k);
 #pragma unroll
 				for (int j = 0; j <= TT; ++j) gw[j] = gw[j] * up;
@@ -1046,7 +1020,14 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 			{
 				// float32: apart from the state's part, which has a scale of its own.  (In half precision a result that is far from its weights is no half.)
 				float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f}, low_sum = sum;
-				if constexpr (HALF) sum = acc[pt] * into[pt];
+				const char* const scales = front + (4 * pt + g) * L::kPitchH + L::kScales;
+				if constexpr (HALF)
+				{
+					// (no infinity for a state that nobody reads)
+					const float4_t worth = *reinterpret_cast<const float4_t*>(scales) * into;
+#pragma unroll
+					for (int r = 0; r < 4; ++r) sum[r] = acc[pt][r] * fminf(worth[r], 0x1p127f);
+				}
 #pragma unroll
 				for (int kk = 0; 2 * kk <= TT; ++kk)
 				{
@@ -1067,10 +1048,12 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				if constexpr (HALF) acc[pt] = sum;
 				else
 				{
+					typedef int Exponents __attribute__((ext_vector_type(4)));
+					const Exponents back_h = *reinterpret_cast<const Exponents*>(scales);
 					sum = add_low(sum, low_sum);
 #pragma unroll
 					for (int r = 0; r < 4; ++r)
-						acc[pt][r] = fmaf(__builtin_amdgcn_ldexpf(acc[pt][r], into_back[pt]), gain, __builtin_amdgcn_ldexpf(sum[r], down_back));
+						acc[pt][r] = fmaf(__builtin_amdgcn_ldexpf(acc[pt][r], back_h[r] + back_c), gain, __builtin_amdgcn_ldexpf(sum[r], back_w));
 				}
 			}
 			if (HALF && scaled)

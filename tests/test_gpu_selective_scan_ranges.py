@@ -142,3 +142,34 @@ def test_the_whole_range_of_float32(ops, scale_x, scale_b, scale_c, seq):
     want, want_state = selective_scan(**args)
     assert relative(y, want) <= F32 and relative(state, want_state) <= F32
     check_scan(y, state, args)
+
+
+@pytest.mark.parametrize("dtype,much", [("f32", 1e10), ("f32", 1e16), ("f32", 1e30), ("f16", 1e6), ("f16", 1e10), ("f16", 1e30)])
+def test_a_loud_state_stays_in_its_row(ops, dtype, much):
+    # an element of a row of the state that nobody reads, far above everything else
+    args = make(dtype, 1, 2, 64, 1, 64, 100)
+    args["c"] = args["c"].clone()
+    args["c"][:, :, 0] = 0.0
+    args["state"][:, :, 3] = 0.0
+    args["state"][:, :, 3, 0] = much
+    args["x"] = args["x"].clone()
+    args["x"][:, :, 3] = 0.0
+    y, state = scan(ops, args)
+    check_scan(y, state, args)
+    assert not y[..., 3].any()
+    want, _ = selective_scan(**args)
+    for p in (0, 2, 4, 15):
+        assert relative(y[..., p], want[..., p]) <= (2.0 ** -10.5 if dtype == "f16" else 2.0 ** -20), p
+
+
+@pytest.mark.parametrize("low", [1e-3, 1e-5, 1e-7])
+def test_quiet_rows_of_the_state_in_float32(ops, low):
+    args = make("f32", 1, 2, 64, 1, 64, 100)
+    args["state"], args["x"] = rows_apart(args["state"], 2, low), rows_apart(args["x"], 2, low)
+    y, state = scan(ops, args)
+    check_scan(y, state, args)
+    want, want_state = selective_scan(**args)
+    # (beside a largest element between 1 and 2^7, as here, an operand is good to 2^-44 at least, which is 2^-44 / low of a row whose values are `low`)
+    for p in range(64):
+        assert relative(y[..., p], want[..., p]) <= F32 + 2.0 ** -44 / low, p
+        assert relative(state[:, :, p], want_state[:, :, p]) <= F32 + 2.0 ** -44 / low, p
