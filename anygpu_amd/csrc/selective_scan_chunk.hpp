@@ -13,10 +13,11 @@
 // The summation index of the results' products is a permuted one (slot 8 g + j of a lane group <-> 16 (j / 4) + 4 g + j % 4), the same in both operands.
 //
 // Half precision: x, B and C are exact.  The weights of the tokens and the state in front of a chunk are rounded to halves, 2^-11 of each term of y, which is
-// what y itself is rounded to; the weights of a token's own tile, which are the largest, keep their remainders.  The state itself stays float32: w x enters
-// as the sum of two halves, 22 bits.  Whether the values that become halves lie where a half has its bits is looked at every time (a maximum and a few lane
-// masks); where they do not, they are brought there by powers of two, which comes out of the sums again.  That path is the slower one by a multiplication per
-// value on either side: the state is kept 2^8 times what it is, which puts common steps and states inside.  The state goes along only as far as it remains a float.
+// what y itself is rounded to: the largest weight of a token and the largest element of a row of the state are brought to the top of a half's range by powers of
+// two, so that this holds down to 2^-29 of them.  The weights of a token's own tile, which are mostly the largest, keep their remainders.  The state itself stays
+// float32: w x enters as the sum of two halves, 22 bits.  Whether these lie where a half has its bits is looked at every time (a maximum and a few lane masks); where
+// they do not, they are brought there in the same way, and the state goes along, as far as it remains a float.  That path is the slower one by a multiplication per
+// value on either side: the state is kept 2^8 times what it is, which puts common steps outside of it.
 // float32: every operand is the sum of two halves, 22 bits and a sign more than a half has, and a product is three (what is left out lies below 2^-22 of it).  The
 // second halves are 2^11 times what they are and their products summed apart, so that they have their bits as far down as the first ones.  x, B
 // and C are scaled by the powers of two that bring a chunk's largest element to the top of a half's range, the state and the weights likewise: all 22 bits down to
@@ -93,13 +94,6 @@ __device__ __forceinline__ int half_exponent(float v, int lowest, int highest)
 constexpr int kLowest = -113, kHighest = 116;       // of the largest float, and of what is a float 2^11 times as large
 
 __device__ __forceinline__ float power_of_two(int k) { return __builtin_bit_cast(float, (127 + k) << 23); }
-
-__device__ __forceinline__ void half_scale(float v, float& up, float& down)
-{
-	const int k = half_exponent(v, kLowest, 58);
-	up = power_of_two(k);
-	down = power_of_two(-k);
-}
 
 // a magnitude that a scale may be taken from: an infinity is beyond all of them, and its neighbours are to keep their bits
 __device__ __forceinline__ float finite_or_zero(float v) { return v < INFINITY ? v : 0.0f; }
@@ -975,32 +969,20 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					most = fmaxf(most, __builtin_fabsf(gw[j][r]));
 				}
 			}
-			int back_c = 0, back_w = 0;                      // float32: exponents of what the products with C and with the weights are worth
-			float into = gain, down = 1.0f;                  // products of the state and C -> those with the weights -> results
-			bool scaled = false;
-			if constexpr (HALF)
-			{
-				// (from 2^-9 on what a column's small weights lose is far below a rounding of its largest)
-				scaled = rows_need_scale(most, 0.001953125f);
-				if (scaled)
-				{
-					float up;
-					half_scale(max_over_lane_rows(most), up, down);
-					into *= up;
-#pragma unroll
-					for (int j = 0; j <= TT; ++j) gw[j] = gw[j] * up;
-				}
-			}
-			else
+			// A column's largest weight, D among them, goes to the top of a half's range: those down to 2^-29 of it keep all their bits.  (Half precision: by 2^22 at
+			// most.  What is lost of a weight then lies below 2^-47, of a result below 64 * 2^16 * 2^-47, half the last bit of the smallest halves; and the scale of a state, 2^105 at
+			// most, remains a float with it.)
+			const int k = half_exponent(max_over_lane_rows(most), kLowest, HALF ? 22 : kHighest);
+			const float up = power_of_two(k), into = gain * up, down = power_of_two(-k);      // half precision: products with C -> those with the weights -> results
+			int back_c = 0, back_w = 0;                                                       // float32: exponents of what either are worth
+			if constexpr (!HALF)
 			{
 				const int* const back = reinterpret_cast<const int*>(steps) + L::kArrays * kChunk;
-				const int k = half_exponent(max_over_lane_rows(most), kLowest, kHighest);
 				back_c = back[L::kBackC];
 				back_w = back[L::kBackX] - k;
-				const float up = power_of_two(k);
-#pragma unroll
-				for (int j = 0; j <= TT; ++j) gw[j] = gw[j] * up;
 			}
+#pragma unroll
+			for (int j = 0; j <= TT; ++j) gw[j] = gw[j] * up;
 			const half4_t none = {};
 			half4_t wf[TT + 1], wl[TT + 1];
 #pragma unroll
@@ -1021,13 +1003,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				// float32: apart from the state's part, which has a scale of its own.  (In half precision a result that is far from its weights is no half.)
 				float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f}, low_sum = sum;
 				const char* const scales = front + (4 * pt + g) * L::kPitchH + L::kScales;
-				if constexpr (HALF)
-				{
-					// (no infinity for a state that nobody reads)
-					const float4_t worth = *reinterpret_cast<const float4_t*>(scales) * into;
-#pragma unroll
-					for (int r = 0; r < 4; ++r) sum[r] = acc[pt][r] * fminf(worth[r], 0x1p127f);
-				}
+				if constexpr (HALF) sum = acc[pt] * (*reinterpret_cast<const float4_t*>(scales) * into);
 #pragma unroll
 				for (int kk = 0; 2 * kk <= TT; ++kk)
 				{
@@ -1045,7 +1021,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					else if (kk == TT / 2) sum = mfma(xf, w_low, sum);
 					sum = mfma(xf, w_hi, sum);
 				}
-				if constexpr (HALF) acc[pt] = sum;
+				if constexpr (HALF) acc[pt] = sum * down;
 				else
 				{
 					typedef int Exponents __attribute__((ext_vector_type(4)));
@@ -1055,11 +1031,6 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					for (int r = 0; r < 4; ++r)
 						acc[pt][r] = fmaf(__builtin_amdgcn_ldexpf(acc[pt][r], back_h[r] + back_c), gain, __builtin_amdgcn_ldexpf(sum[r], back_w));
 				}
-			}
-			if (HALF && scaled)
-			{
-#pragma unroll
-				for (int pt = 0; pt < PT; ++pt) acc[pt] = acc[pt] * down;
 			}
 			before_stores();
 			if (t0 + t < end)

@@ -469,8 +469,9 @@ int anygpu_causal_conv1d_silu_chunk_f32(const float* x, float* state, const floa
  * state: float32 [batch, heads, head_dim, state_dim], dense, read as the state in front of the first token and overwritten
  * with the one behind the last; NULL: from zeros, not kept.  lengths as above: tokens behind a row's length make no step and
  * their y is zeros.  Steps, sums along the sequence and states are float32 or wider; in the half precision form the weights
- * of the tokens and the state that a chunk of 64 tokens starts from enter the matrix products as halves of their own scale,
- * and states are kept 2^8 times what they are (magnitudes up to 2^119 = 6e35).
+ * of the tokens and the state that a chunk of 64 tokens starts from enter the matrix products as halves: good to 2^-11 of
+ * themselves down to 2^-29 of a token's largest weight (D is one of its own) and of the largest element of a row of the state.
+ * States are kept 2^8 times what they are there (magnitudes up to 2^119 = 6e35).
  * In the float32 form every operand enters as the sum of two halves, scaled by the largest finite element of a head's x, of B or
  * of C in the chunk: good to 2^-22 of itself down to 2^-29 of that largest element (down to 2^-22 where the largest lies between
  * 1 and 128), below that to 2^-44 of the largest; the same holds for the weights of one token (B . C times its decay times its

@@ -173,3 +173,19 @@ def test_quiet_rows_of_the_state_in_float32(ops, low):
     for p in range(64):
         assert relative(y[..., p], want[..., p]) <= F32 + 2.0 ** -44 / low, p
         assert relative(state[:, :, p], want_state[:, :, p]) <= F32 + 2.0 ** -44 / low, p
+
+
+@pytest.mark.parametrize("step,much", [(1e-6, 100.0), (1e-5, 30.0), (1e-6, 1.0), (1e-4, 1000.0)])
+@pytest.mark.parametrize("seq", [16, 64, 100])
+def test_weights_far_below_the_skip_term_in_half_precision(ops, step, much, seq):
+    # D of one on a token's own place, weights of a millionth for the others, and channels where the token itself has nothing: those see only the small weights
+    args = make("f16", 1, 2, 64, 1, 64, seq, carried=False)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seq)
+    x = torch.empty(1, 2, 64, seq, device="cuda").normal_(generator=gen) * much
+    x[..., 1::2] *= (torch.rand(1, 2, 64, x[..., 1::2].shape[-1], device="cuda", generator=gen) < 0.5)
+    x[:, :, :32, seq // 2:] = 0.0
+    args.update(x=x.half(), skip=torch.ones(2, device="cuda"), bias=torch.full((2,), math.log(math.expm1(step)), device="cuda"), dt=torch.zeros_like(args["dt"]),
+                b=(args["b"].float().abs() * 0.3 + 0.3).half(), c=(args["c"].float().abs() * 0.3 + 0.3).half(), state=torch.zeros(1, 2, 64, 64, device="cuda"))
+    y, state = scan(ops, args)
+    check_scan(y, state, args)
