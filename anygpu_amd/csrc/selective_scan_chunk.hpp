@@ -871,14 +871,10 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 			x_at[k] = l * L::kPitchX + (16 * k + 4 * g) * 2;
 			asm volatile("" : "+v"(x_at[k]));
 		}
-		// in a token's own tile: nothing of the tokens behind it, D for itself
-		float4_t behind, itself;
+		// in a token's own tile: D for itself (nothing of the tokens behind it, whatever they are)
+		float4_t itself;
 #pragma unroll
-		for (int r = 0; r < 4; ++r)
-		{
-			behind[r] = 4 * g + r > l ? -INFINITY : 0.0f;
-			itself[r] = 4 * g + r == l ? (HALF ? skip : 1.0f) : 0.0f;
-		}
+		for (int r = 0; r < 4; ++r) itself[r] = 4 * g + r == l ? (HALF ? skip : 1.0f) : 0.0f;
 		const auto chunk = [&](auto which, int t0, int turn, auto before_stores) {
 			constexpr int TT = decltype(which)::value;
 			const char* const ops = lds + (DOUBLE ? turn * L::kStage : 0);
@@ -959,13 +955,14 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					const float4_t from = *reinterpret_cast<const float4_t*>(steps + (HALF ? L::kFrom : L::kIn) * kChunk + s);
 					const float4_t low = *reinterpret_cast<const float4_t*>(steps + (HALF ? L::kFromLow : L::kInLow) * kChunk + s);
 #pragma unroll
-					for (int r = 0; r < 4; ++r) e[r] = fast_exp2((in - from[r]) + ((in_low - low[r]) + behind[r]));
+					for (int r = 0; r < 4; ++r) e[r] = fast_exp2((in - from[r]) + (in_low - low[r]));
 				}
 				if constexpr (!HALF) e = e * (*reinterpret_cast<const float4_t*>(steps + L::kDelta * kChunk + s) * steps[L::kArrays * kChunk + L::kScaleBC]);
 #pragma unroll
 				for (int r = 0; r < 4; ++r)
 				{
-					gw[j][r] = j == TT ? fmaf(gw[j][r], e[r], HALF ? itself[r] : itself[r] * own) : gw[j][r] * e[r];
+					if (j < TT) gw[j][r] = gw[j][r] * e[r];
+					else gw[j][r] = 4 * g + r > l ? 0.0f : fmaf(gw[j][r], e[r], HALF ? itself[r] : itself[r] * own);
 					most = fmaxf(most, __builtin_fabsf(gw[j][r]));
 				}
 			}

@@ -374,8 +374,8 @@ def tensor_selective_scan(xt: torch.Tensor, dt: torch.Tensor, at: torch.Tensor, 
     state, float32 [batch, heads, head_dim, state_dim]: the state in front of the first token, updated in place; None starts from zeros.
     lengths (int32 [batch], on the device): tokens of each row of a padded batch; y behind them is zeros.
     state_dim is at most 256.  Other tensors must not share memory with state.
-    The matrix products take their operands as halves, or as pairs of halves in float32 (22 bits, scaled by the largest value of 64 tokens); a value
-    that is not finite may also reach results of the 63 tokens in front of it."""
+    The matrix products take their operands as halves, or as pairs of halves in float32 (22 bits, scaled by the largest value of 64 tokens); an x
+    that is not finite may also reach results of the 63 tokens in front of it in its row."""
     got = (_native or _calls()).selective_scan(xt, dt, at, bt, ct, dt_bias, skip, state, lengths, dt_limit[0], dt_limit[1])
     if got is not None:
         return got

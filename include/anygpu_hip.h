@@ -479,8 +479,8 @@ int anygpu_causal_conv1d_silu_chunk_f32(const float* x, float* state, const floa
  * token more than 2^29 times as large as others costs these bits, also those in front of it in the chunk.  A decay since a
  * chunk's start below 2^-126 counts as none.  The whole range of floats is taken; where B and C are both small, elements of 1e-15
  * and less (1e-30 where the other one is about one) are not brought up any further.
- * A value that is not finite reaches the results behind it as in the formula above, and besides may reach those of up to 63
- * tokens in front of it (of its row, for x and the state's rows; of its group's heads, for B and C).
+ * A value that is not finite reaches the results behind it as in the formula above; one of x may besides reach those of up to 63
+ * tokens in front of it in its row.
  * state_dim <= ANYGPU_SCAN_MAX_STATE.  workspace: device memory, 16-byte aligned, of at least
  * anygpu_selective_scan_workspace_bytes (0 for many shapes; a negative error code for shapes that are rejected), for the
  * states of long sequences that are shared out over blocks; the next call on the same stream may reuse it, calls that may

@@ -189,3 +189,32 @@ def test_weights_far_below_the_skip_term_in_half_precision(ops, step, much, seq)
                 b=(args["b"].float().abs() * 0.3 + 0.3).half(), c=(args["c"].float().abs() * 0.3 + 0.3).half(), state=torch.zeros(1, 2, 64, 64, device="cuda"))
     y, state = scan(ops, args)
     check_scan(y, state, args)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("key,value", [("b", math.inf), ("b", math.nan), ("c", -math.inf), ("c", math.nan), ("dt", math.nan), ("dt", math.inf)])
+@pytest.mark.parametrize("seq", [70, 1500])
+def test_what_is_not_finite_in_b_c_and_dt_stays_behind_its_token(ops, dtype, key, value, seq):
+    at = seq - 30
+    args = make(dtype, 1, 4, 64, 2, 64, seq)
+    want, want_state = selective_scan(**args)
+    odd = {**args, key: args[key].clone()}
+    if key == "dt":
+        odd["dt"][0, 1, at] = value
+    else:
+        odd[key][0, 0, 5, at] = value
+    y, state = scan(ops, odd)
+    # heads 0 and 1 share the first group, head 1 has the step
+    hit = [1] if key == "dt" else [0, 1]
+    assert not torch.isfinite(y[0, at, hit]).any()
+    if key != "c":
+        assert not torch.isfinite(y[0, at:, hit]).any()
+        assert not torch.isfinite(state[0, hit] if key == "dt" else state[0, hit, :, 5]).any()
+    # all else is what it is without it: put that in where it belongs, and compare everything
+    for h in hit:
+        y[0, at if key == "c" else slice(at, None), h] = want[0, at if key == "c" else slice(at, None), h].to(y)
+        if key == "dt":
+            state[0, h] = want_state[0, h].to(state)
+        elif key == "b":
+            state[0, h, :, 5] = want_state[0, h, :, 5].to(state)
+    check_scan(y, state, args)
