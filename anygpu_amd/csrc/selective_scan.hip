@@ -2,7 +2,7 @@
 //     H_t = exp(delta_t A) H_{t-1} + delta_t x_t B_t^T,   y_t = H_t C_t + D x_t
 // In chunks of 64 tokens on the matrix cores (selective_scan_chunk.hpp); here are the plan of such a launch, and the scan token by token for what the chunks' kernel
 // does not take, rows of x, B or C that lie gigabytes apart: a wave has a row of H (one of head_dim), four elements of the state a lane, in registers for the whole
-// sequence, and every token waits for its operands (2 x 2048 tokens, 32 heads, state 256, float32: 13.8 ms, in chunks 164 us).
+// sequence, and every token waits for its operands (2 x 2048 tokens, 32 heads, state 256, float32: 13.8 ms, in chunks 140 us).
 #include "selective_scan.hpp"
 #include "selective_scan_chunk.hpp"
 #include "launch.hpp"
@@ -75,14 +75,14 @@ hipError_t launch_token(const ScanArgs& a, hipStream_t stream)
 	return hipGetLastError();
 }
 
-// Rows of a block: heads of 32 rows take blocks of 32 (4 x 4096 tokens, 64 heads, f16 86 us, in half empty blocks of 64 121; heads of 64 in two blocks of
-// 32: 164 against 93, twice the weights and twice the fetching of B and C).
+// Rows of a block: heads of 32 rows take blocks of 32 (4 x 4096 tokens, 64 heads, f16 78 us, in half empty blocks of 64 88; heads of 64 in two blocks of
+// 32: 157 against 90, twice the weights and twice the fetching of B and C).
 // Segments: sequences whose blocks leave compute units without work are cut, in pieces of four chunks at least.  The pass that finds the segments'
 // states costs about half of the other one, so that two blocks on a compute unit (the half precision form up to a state of 64) pay from three segments on, one
-// from two on (16384 tokens, 128 heads, f16: uncut 312 us, 4 segments 256, 8 283; 3 x 4096 tokens, 64 heads, f16: uncut 85, 2 segments 101; 2 x 2048 tokens, 64 heads,
-// f32: 87, 2 segments 72; one such sequence 82, 4 segments 48, 8 58), and that short sequences stay whole (500 tokens, 64 heads, f16: 17 us, cut 19).  The first pass takes half a segment per block where all its blocks are then
-// still resident at once (16000 tokens, 128 heads, f16: 236 us whole, 223 in halves, 226 in thirds; 3 x 1001 tokens, 32 heads, state 128, f32: 80, 70, 79; where they
-// are not, 8192 tokens, 2 x 32 heads, f16: 69, 74).
+// from two on (16384 tokens, 128 heads, f16: uncut 328 us, 4 segments 253, 8 285; 3 x 4096 tokens, 64 heads, f16: uncut 84, 2 segments 97; 2 x 2048 tokens, 64 heads,
+// f32: 82, 2 segments 69; one such sequence 81, 4 segments 47, 8 57), and that short sequences stay whole (500 tokens, 64 heads, f16: 15.0 us, cut 15.9; f32 27.6, 26.1).  The first pass takes half a segment per block where all its blocks are then
+// still resident at once (16000 tokens, 128 heads, f16: 245 us whole, 231 in halves; 3 x 1001 tokens, 32 heads, state 128, f32: 72, 64; where they
+// are not, 8192 tokens, 2 x 32 heads, f16: 67, 68).
 scan::Plan make_plan(bool half, int64_t batch, int64_t heads, int64_t head_dim, int64_t state_dim, int64_t seqlen)
 {
 	scan::Plan plan{};

@@ -21,14 +21,14 @@
 // float32: every operand is the sum of two halves, 22 bits and a sign more than a half has, and a product is three (what is left out lies below 2^-22 of it).  The
 // second halves are 2^11 times what they are and their products summed apart, so that they have their bits as far down as the first ones.  x, B
 // and C are scaled by the powers of two that bring a chunk's largest element to the top of a half's range, the state and the weights likewise: all 22 bits down to
-// 2^-29 of the largest, 2^-51 of the largest below that.  Sums are float32, and powers of two come out of them by exponents.  The fp32 matrix instruction does a sixteenth of what the one for halves does in its time (4 x 4096 tokens, 64 heads: 292 us with it, 194 with halves).
+// 2^-29 of the largest, 2^-51 of the largest below that.  Sums are float32, and powers of two come out of them by exponents.  The fp32 matrix instruction does a sixteenth of what the one for halves does in its time (4 x 4096 tokens, 64 heads: 292 us with it in an early form of this kernel, 236 with halves then, 200 now).
 // Steps are summed in 64 bits, and the distance of two tokens is put together from pieces of one sign - from a token to its tile's edge, tile by tile, and
 // from an edge to a token - so that no difference of long sums is taken; inside a tile the sums are pairs of floats.
 //
-// Measured (heads of 64 rows, state 64; the bytes are x, B, C, dt, y and the states once): 4 x 4096 tokens, 64 heads, half precision 92 - 98 us = 2.8 - 3.0 TB/s, 16 x 1024 tokens 79,
-// 16384 tokens, 128 heads 250 us = 2.2 TB/s, of which 80 are the first pass; float32 4 x 4096 tokens 194 us = 2.8 TB/s.  What bounds it, at one block of 8 waves on a
-// CU as at two: the same loads and stores alone take 71 us (rows of 128 bytes, 8 KB apart), all the rest alone 87; the vector units issue 0.43 of the cycles
-// (1240 instructions a chunk and block), the matrix units are busy 0.21 of them, with two blocks 0.49 and 0.25.  Two chunks ahead with the loads, one with the LDS, hides most of either behind the other.
+// Measured (heads of 64 rows, state 64; the bytes are x, B, C, dt, y and the states once): 4 x 4096 tokens, 64 heads, half precision 96 - 106 us = 2.6 - 2.9 TB/s, 16 x 1024 tokens 85,
+// 16384 tokens, 128 heads 253 us = 2.2 TB/s, of which 80 are the first pass; float32 4 x 4096 tokens 200 us = 2.7 TB/s.  What bounds it, at one block of 8 waves on a
+// CU as at two: the same loads and stores alone take 71 us (rows of 128 bytes, 8 KB apart), all the rest alone 89; the vector units issue 0.51 of the cycles
+// (1570 instructions a chunk and block), the matrix units are busy 0.20 of them, with two blocks 0.61 and 0.24.  Two chunks ahead with the loads, one with the LDS, hides most of either behind the other.
 #pragma once
 
 #include "launch.hpp"
@@ -69,7 +69,7 @@ struct Lds
 	// two chunks' operands where that leaves room for as many blocks as the registers do (half precision: two, three without results) or does not matter
 	static constexpr int kBlocks = kHalf && NT <= 64 ? (STATES ? 3 : 2) : 1;
 	// float32, where fetching and splitting the operands is as much work as the state's: a trade of its own, where the registers leave room for its waves
-	// (4 x 4096 tokens, 64 heads: 236 us without, 194 with; 3 x 1001 tokens, 32 heads, state 128, whose first pass only has it: 3 % less)
+	// (4 x 4096 tokens, 64 heads: 247 us without, 206 with; 3 x 1001 tokens, 32 heads, state 128, whose first pass only has it: 4 % less)
 	static constexpr bool kMovers = !kHalf && (NT <= 64 || STATES);
 	static constexpr int kThreads = 4 * R * (kMovers ? 2 : 1) + (STATES ? 0 : 256), kWaves = (kThreads / 64 * kBlocks + 3) / 4;        // (of a SIMD)
 	static constexpr int kStages = kBlocks * (2 * kStage + 2 * kFront + kTwoSteps) <= 160 * 1024 ? 2 : 1;
@@ -410,8 +410,8 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 			}
 			// (a scalar base and a lane's 32-bit offset, not six 64-bit pointers that are carried along in vector registers)
 			asm volatile("" : "+s"(t0));
-			// (plain loads also of x, which is read once or, by two passes, twice: non-temporal ones 64 us instead of 59 for 3 x 1001 tokens, state 128, float32, 24.9
-			// and 23.6 for 700, f16, and nothing to 3 % less for what no cache holds)
+			// (plain loads also of x, which is read once or, by two passes, twice: non-temporal ones 72 us instead of 67 for 3 x 1001 tokens, state 128, float32, 29.1
+			// and 27.2 for 500, and within 2 % of each other for what no cache holds)
 #pragma unroll
 			for (int i = 0; i < XV; ++i) o.x[i] = *fetch(x + t0, xo[i]);
 			if constexpr (AHEAD)
@@ -420,7 +420,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				for (int i = 0; i < BA; ++i) o.b[i] = *fetch(b + t0, bo[i]);
 				if constexpr (!STATES)
 				{
-					// (float32 without waves that only fetch: 256 registers are all there are, and C's offsets are made afresh - 66.5 us instead of 68.2 with a spilled pair of them
+					// (float32 without waves that only fetch: 256 registers are all there are, and C's offsets are made afresh - 66.5 us, 68.2 with a spilled pair of them
 					// for 3 x 1001 tokens, 32 heads, state 128)
 					unsigned c_row = (unsigned)a.c_row;
 					if constexpr (!HALF && !MOVERS) asm volatile("" : "+s"(c_row));
@@ -584,7 +584,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 		if (MOVERS && moves)
 		{
 			// Two chunks under way: a chunk's loads have the time of two until they are waited for, and nobody waits for them while another is split (4 x 4096 tokens,
-			// 64 heads: 233 us with one, 198 with two)
+			// 64 heads: 233 us with one, 198 with two, before the second halves had a scale of their own)
 			Operands even, odd;
 			if (begin < end)
 			{

@@ -4,7 +4,8 @@
  *
  * Conventions
  *   - every pointer is a DEVICE pointer into memory the caller owns; inputs are only read,
- *     outputs only written.  One kind of scratch exists: the GEMM entry points cut some products
+ *     outputs only written.  Beside the workspaces that are arguments (decode attention, selective
+ *     scan), one kind of scratch exists: the GEMM entry points cut some products
  *     along K (few tiles and a deep K, few rows against a weight matrix) and pass the partial
  *     sums of such a launch through a workspace that belongs to the (device, stream) pair of the
  *     call; the same workspace takes the aligned copy of a GEMM operand that cannot be fetched
