@@ -218,3 +218,27 @@ def test_what_is_not_finite_in_b_c_and_dt_stays_behind_its_token(ops, dtype, key
         elif key == "b":
             state[0, h, :, 5] = want_state[0, h, :, 5].to(state)
     check_scan(y, state, args)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("quiet", [1e-2, 1e-4, 1e-5])
+@pytest.mark.parametrize("seq", [40, 64, 150])
+def test_a_loud_token_beside_quiet_ones_in_a_row_of_the_state(ops, dtype, quiet, seq):
+    # the loud one meets B in one half of the state, the quiet ones in the other: each half has its own errors, but the products are made with one scale
+    args = make(dtype, 1, 2, 64, 1, 64, seq, carried=False)
+    args["x"], args["b"] = args["x"] * quiet, args["b"].clone()
+    args["x"][..., 9] *= 1.0 / quiet
+    args["b"][:, :, :32] = 0.0
+    args["b"][:, :, :, 9] = 0.0
+    args["b"][:, :, :32, 9] = 1.0
+    args.update(a=torch.full((2,), -1e-3, device="cuda"), bias=torch.full((2,), -4.0, device="cuda"), dt=torch.zeros_like(args["dt"]), state=torch.zeros(1, 2, 64, 64, device="cuda"))
+    _, state = scan(ops, args)
+    _, want = selective_scan(**args)
+    _, mag = magnitudes(**args)
+    # as in check_scan; and what is lost of step times x below the largest of a row: 2^-21 of it, in float32 2^-51, for every token (decays are next to one)
+    step = math.log1p(math.exp(-4.0))
+    lost = (2.0 ** -21 if dtype == "f16" else 2.0 ** -51) * step * args["x"].double().abs().amax(dim=3)[..., None] * args["b"].double().abs().sum(3)[:, :, None]
+    assert float(((state.double() - want).abs() / ((4 * seq + 64 + 16) * 2.0 ** -24 * mag + lost + 1e-37)).max()) <= 1.0
+    assert relative(state[..., :32], want[..., :32]) <= 2.0 ** -20
+    if dtype == "f32":
+        assert relative(state[..., 32:], want[..., 32:]) <= 2.0 ** -20
