@@ -375,8 +375,8 @@ def tensor_selective_scan(xt: torch.Tensor, dt: torch.Tensor, at: torch.Tensor, 
     lengths (int32 [batch], on the device): tokens of each row of a padded batch; y behind them is zeros.
     state_dim is at most 256.  Other tensors must not share memory with state.
     The matrix products take their operands as halves, or as pairs of halves in float32, which are scaled by the largest element of a chunk of 64 tokens and keep
-    all of their bits (22 in float32) down to 2^-29 of it, below that 2^-44 of the largest: a finite value more than 5e8 times as large as others may cost those
-    their last bits, also 63 tokens in front of it.  An x that is not finite may also reach results of the 63 tokens in front of it in its row.
+    all of their bits (22 in float32) down to 2^-29 of it, or down to 2^-22 where it lies between 1 and 128: a finite value more than 5e8 times as large as
+    others may cost those their last bits, also 63 tokens in front of it.  An x that is not finite may also reach results of the 63 tokens in front of it in its row.
     tensor_selective_scan_update works in float32 throughout.  float16 keeps states up to 6e35."""
     got = (_native or _calls()).selective_scan(xt, dt, at, bt, ct, dt_bias, skip, state, lengths, dt_limit[0], dt_limit[1])
     if got is not None:

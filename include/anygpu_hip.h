@@ -476,7 +476,7 @@ int anygpu_causal_conv1d_silu_chunk_f32(const float* x, float* state, const floa
  * States are kept 2^8 times what they are there (magnitudes up to 2^119 = 6e35).
  * In the float32 form every operand enters as the sum of two halves, scaled by the largest finite element of a head's x, of B or
  * of C in the chunk: good to 2^-22 of itself down to 2^-29 of that largest element (down to 2^-22 where the largest lies between
- * 1 and 128), below that to 2^-44 of the largest; the same holds for the weights of one token (B . C times its decay times its
+ * 1 and 128), below that to 2^-50 of the largest (2^-44 where it lies there); the same holds for the weights of one token (B . C times its decay times its
  * step), step times x in a row, and a row of the state in front of a chunk.  So a finite
  * token more than 2^29 times as large as others costs these bits, also those in front of it in the chunk.  A decay since a
  * chunk's start below 2^-126 counts as none.  The whole range of floats is taken; where B and C are both small, elements of 1e-15

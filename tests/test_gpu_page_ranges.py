@@ -35,3 +35,24 @@ def test_an_empty_source_inside_of_a_written_cache(ops):
                                        one(ctypes.c_int64, 0), 1, to.data_ptr(), origin.data_ptr(), 2, torch.cuda.current_stream().cuda_stream)
     assert rc == capi.ANYGPU_OK
     assert not pages[1].any() and pages[2, 0] == 8
+
+
+@pytest.mark.parametrize("moves,pages", [(5000, 12000), (20000, 60000), (3000, 90000), (4097, 4200)])
+@pytest.mark.parametrize("apart", [True, False])
+def test_lists_of_thousands_of_moves(ops, moves, pages, apart):
+    gen = torch.Generator().manual_seed(moves)
+    cache = torch.randn(pages, 12, generator=gen)
+    if apart:
+        order = torch.randperm(pages, generator=gen)
+        to = order[:min(moves, pages // 2)]
+        origin = order[len(to):][torch.randint(0, pages - len(to), (len(to),), generator=gen)]
+        origin[::7] = -1
+    else:
+        to, origin = (torch.randint(-1, pages + 1, (moves,), generator=gen) for _ in range(2))
+    want = cache.clone()
+    for t, f in zip(to.tolist(), origin.tolist()):
+        if 0 <= t < pages and -1 <= f < pages:
+            want[t] = want[f].clone() if f >= 0 else 0.0
+    got = cache.cuda()
+    ops.tensor_copy_pages(got, got, to.int().cuda(), origin.int().cuda())
+    assert torch.equal(got.cpu(), want)
