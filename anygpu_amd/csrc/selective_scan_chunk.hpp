@@ -21,7 +21,8 @@
 // float32: every operand is the sum of two halves, 22 bits and a sign more than a half has, and a product is three (what is left out lies below 2^-22 of it).  The
 // second halves are 2^11 times what they are and their products summed apart, so that they have their bits as far down as the first ones.  x, B
 // and C are scaled by the powers of two that bring a chunk's largest element to the top of a half's range, the state and the weights likewise: all 22 bits down to
-// 2^-29 of the largest, 2^-51 of the largest below that.  Sums are float32, and powers of two come out of them by exponents.  The fp32 matrix instruction does a sixteenth of what the one for halves does in its time (4 x 4096 tokens, 64 heads: 292 us with it in an early form of this kernel, 236 with halves then, 200 now).
+// 2^-29 of the largest, 2^-51 of the largest below that.  Sums are float32, and powers of two come out of them by exponents.  The fp32 matrix instruction does a
+// sixteenth of what the one for halves does in its time (4 x 4096 tokens, 64 heads: 292 us with it in an early form of this kernel, 236 with halves then, 200 now).
 // Steps are summed in 64 bits, and the distance of two tokens is put together from pieces of one sign - from a token to its tile's edge, tile by tile, and
 // from an edge to a token - so that no difference of long sums is taken; inside a tile the sums are pairs of floats.
 //
@@ -1026,7 +1027,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					sum = add_low(sum, low_sum);
 #pragma unroll
 					for (int r = 0; r < 4; ++r)
-						acc[pt][r] = fmaf(__builtin_amdgcn_ldexpf(acc[pt][r], back_h[r] + back_c), gain, __builtin_amdgcn_ldexpf(sum[r], back_w));
+						acc[pt][r] = __builtin_amdgcn_ldexpf(acc[pt][r] * gain, back_h[r] + back_c) + __builtin_amdgcn_ldexpf(sum[r], back_w);      // (decayed first: the products of a large state may be no floats)
 				}
 			}
 			before_stores();

@@ -242,3 +242,19 @@ def test_a_loud_token_beside_quiet_ones_in_a_row_of_the_state(ops, dtype, quiet,
     assert relative(state[..., :32], want[..., :32]) <= 2.0 ** -20
     if dtype == "f32":
         assert relative(state[..., 32:], want[..., 32:]) <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("size", [64, 128, 200])
+def test_a_state_whose_products_with_c_are_floats_only_once_it_has_decayed(ops, size):
+    args = make("f32", 1, 2, 64, 1, size, 70)
+    args["state"], args["c"] = args["state"].clamp(-2.0, 2.0) * 1e37, args["c"] * 1e4
+    args["a"], args["bias"], args["dt"] = torch.full((2,), -8.0, device="cuda"), torch.full((2,), 1.0, device="cuda"), torch.zeros_like(args["dt"])
+    y, state = scan(ops, args)
+    want, want_state = selective_scan(**args)
+    mag, mag_state = magnitudes(**args)
+    assert float(mag.max()) < 3e38 and torch.isfinite(y).all()
+    # (decays below 2^-126 since the chunk's start count as none: see above)
+    undecayed = (args["state"].double().abs()[:, :, :, :, None] * args["c"].double().abs()[:, :, None]).sum(3).permute(0, 3, 1, 2)
+    f32 = (4 * 70 + size + 16) * 2.0 ** -24
+    assert float(((y.double() - want).abs() / (f32 * mag + 2.0 ** -126 * undecayed)).max()) <= 1.0
+    assert float(((state.double() - want_state).abs() / (f32 * mag_state + 2.0 ** -126 * args["state"].double().abs())).max()) <= 1.0
