@@ -958,7 +958,12 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 #pragma unroll
 					for (int r = 0; r < 4; ++r) e[r] = fast_exp2((in - from[r]) + (in_low - low[r]));
 				}
-				if constexpr (!HALF) e = e * (*reinterpret_cast<const float4_t*>(steps + L::kDelta * kChunk + s) * steps[L::kArrays * kChunk + L::kScaleBC]);
+				if constexpr (!HALF)
+				{
+					// (the smallest and the largest steps last: their products with the scale alone may be no floats)
+					gw[j] = gw[j] * (e * steps[L::kArrays * kChunk + L::kScaleBC]);
+					e = *reinterpret_cast<const float4_t*>(steps + L::kDelta * kChunk + s);
+				}
 #pragma unroll
 				for (int r = 0; r < 4; ++r)
 				{

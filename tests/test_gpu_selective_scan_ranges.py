@@ -258,3 +258,14 @@ def test_a_state_whose_products_with_c_are_floats_only_once_it_has_decayed(ops, 
     f32 = (4 * 70 + size + 16) * 2.0 ** -24
     assert float(((y.double() - want).abs() / (f32 * mag + 2.0 ** -126 * undecayed)).max()) <= 1.0
     assert float(((state.double() - want_state).abs() / (f32 * mag_state + 2.0 ** -126 * args["state"].double().abs())).max()) <= 1.0
+
+
+@pytest.mark.parametrize("step", [1e-20, 1e-30, 1e-33, 1e25])
+@pytest.mark.parametrize("size", [64, 128])
+def test_steps_far_from_one_in_float32(ops, step, size):
+    # nothing but what such steps bring in: no state, no D (and next to no decay)
+    args = make("f32", 1, 2, 64, 1, size, 130, carried=False)
+    args.update(skip=None, state=torch.zeros(1, 2, 64, size, device="cuda"), a=torch.full((2,), -1e-3 / max(step, 1.0), device="cuda"), limit=(step, step))
+    y, state = scan(ops, {k: v for k, v in args.items() if k != "limit"}, dt_limit=(step, step))
+    want, want_state = selective_scan(**args)
+    assert relative(y, want) <= F32 and relative(state, want_state) <= F32
