@@ -718,7 +718,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 					for (int i = 0; i < NB; ++i)
 #pragma unroll
 						for (int r = 0; r < 4; ++r) largest = fmaxf(largest, __builtin_fabsf(h[i][r]));
-					const int k_most = half_exponent(max_over_lane_rows(most), kLowest, 58),
+					const int k_most = half_exponent(max_over_lane_rows(most), kLowest, kHighest),
 					          room = 252 - ((__builtin_bit_cast(int, max_over_lane_rows(largest)) >> 23) & 255), k = k_most < room ? k_most : room;
 					const float up = power_of_two(k);
 					into *= up;

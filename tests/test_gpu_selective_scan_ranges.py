@@ -269,3 +269,14 @@ def test_steps_far_from_one_in_float32(ops, step, size):
     y, state = scan(ops, {k: v for k, v in args.items() if k != "limit"}, dt_limit=(step, step))
     want, want_state = selective_scan(**args)
     assert relative(y, want) <= F32 and relative(state, want_state) <= F32
+
+
+@pytest.mark.parametrize("step", [1e-20, 1e-27, 1e-30, 1e-33])
+@pytest.mark.parametrize("size,seq", [(64, 130), (128, 40), (250, 70), (64, 1500)])
+def test_small_steps_reach_the_state_in_half_precision(ops, step, size, seq):
+    args = make("f16", 1, 2, 64, 1, size, seq, carried=False)
+    args.update(state=torch.zeros(1, 2, 64, size, device="cuda"), a=torch.full((2,), -1e-3, device="cuda"), limit=(step, step))
+    y, state = scan(ops, {k: v for k, v in args.items() if k != "limit"}, dt_limit=(step, step))
+    check_scan(y, None, args)
+    _, want = selective_scan(**args)
+    assert relative(state, want) <= 2.0 ** -20
