@@ -937,6 +937,9 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 			// ---- weights: G exp(L_t - L_s) delta_s, the skip term on the diagonal ----
 			const float in = steps[L::kIn * kChunk + t], in_low = steps[L::kInLow * kChunk + t], gain = steps[L::kGain * kChunk + t];
 			const float own = HALF ? 1.0f : steps[L::kArrays * kChunk + L::kSkip];
+			// (float32 without waves that only fetch: compared anew in every chunk, for the masks would take eight scalar registers that there are not)
+			int later = 4 * g;
+			if constexpr (!HALF && !MOVERS) asm volatile("" : "+v"(later));
 			float since = in;                                // from the end of the tile j to the token
 			float most = 0.0f;
 #pragma unroll
@@ -968,7 +971,7 @@ __global__ __launch_bounds__((Lds<T, NT, R, STATES>::kThreads), (Lds<T, NT, R, S
 				for (int r = 0; r < 4; ++r)
 				{
 					if (j < TT) gw[j][r] = gw[j][r] * e[r];
-					else gw[j][r] = 4 * g + r > l ? 0.0f : fmaf(gw[j][r], e[r], HALF ? itself[r] : itself[r] * own);
+					else gw[j][r] = later + r > l ? 0.0f : fmaf(gw[j][r], e[r], HALF ? itself[r] : itself[r] * own);
 					most = fmaxf(most, __builtin_fabsf(gw[j][r]));
 				}
 			}
